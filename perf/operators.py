@@ -15,7 +15,6 @@ int8, scales fp32 ``[pages, heads]``, page means of the key codes int8 ``[pages,
 """
 from __future__ import annotations
 
-import functools
 import importlib
 import math
 
@@ -258,7 +257,6 @@ def run(s):
     return {"norms": _plain_norms, "cache": _plain_cache, "attend": _plain_attend, "select": _plain_select}[kind](s)
 
 
-@functools.lru_cache(maxsize=None)
 def _module(name):
     return importlib.import_module(f"{PACKAGE}.{name}")
 
