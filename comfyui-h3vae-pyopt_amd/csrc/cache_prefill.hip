@@ -13,8 +13,9 @@
 //                      other without leaving its lane.
 //
 // The page's value scale s_v = f * 2^e, f in [1/2, 1): f joins the weights (exp2(x + log2 f), the row sum takes 1 / f
-// back), 2^e the codes, relative to the largest e so far, so that both stay exact powers of two away from the codes and
-// the accumulators need no pass of their own; where a larger e turns up they are scaled down to it.
+// back), 2^e the codes, relative to a reference that the accumulators have too: the largest e so far.  fp16 holds codes
+// down to 2^-24 of it exactly.  A page further below has a reference of its own, 24 above its e, and the accumulators are brought
+// to it before its product and back after it: a power of two each way, exact since fp32 has room for both.
 //
 // One barrier per step.  On each SIMD a wave of the first half of the workgroup meets one of the second, and their order of
 // work is such that the softmax of one runs beside the products of the other: with two sets of 32 rows (QS = 2) the first half
@@ -48,7 +49,7 @@ __device__ __forceinline__ int swz(int row, int chunk) {
     else return chunk ^ (row & 15);
 }
 
-// fp16 values of 8 codes times `f` (a power of two), exactly: (1024 + byte) f - 1152 f
+// fp16 values of 8 codes times `f` (a power of two from 2^-24 on, or 0), exactly: (1024 + byte) f - 1152 f, with off = -1152 f
 __device__ __forceinline__ u32x4 scaled_codes(uint32_t w0, uint32_t w1, f16x2 f, f16x2 off) {
     const uint32_t u0 = w0 ^ 0x80808080u, u1 = w1 ^ 0x80808080u;
     const uint32_t a[4] = {__builtin_amdgcn_perm(0x64646464u, u0, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, u0, 0x04030402u),
@@ -62,12 +63,17 @@ __device__ __forceinline__ u32x4 scaled_codes(uint32_t w0, uint32_t w1, f16x2 f,
 
 // One page's part of a step: its id (-1: not there) and scales.  A value scale of zero (its codes are) or a bad scale (infinite
 // or NaN: the scores of the rows that see the page become NaN) stands as a harmless number.
+constexpr float kNoScale = 1.0e-37f;
 struct Part {
     int id;
     float ks, vs;
     bool bad;
-    int e;        // the largest value exponent up to this page
+    int e;        // the reference exponent of its codes and of the accumulators
 };
+
+// Codes are exact down to 2^-24 of the reference.  It drops by at most 75: accumulators stay below 2^(kLazy + kLift) * 127 * 2^30 keys
+// < 2^52 of the largest value scale so far, and so below 2^127.  The values of a page below 2^-99 of that scale count as zeros.
+constexpr int kExact = 24, kDrop = 75;
 
 // The item-th tile of `rows` rows of the sequences that are long, a sequence's last tiles first; false behind the last.
 __device__ __forceinline__ bool long_tile(const AttnParams& p, int rows, int item, int& b, int& tile) {
@@ -214,8 +220,10 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
             r.vs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, pg_vs), n));
             r.bad = !(r.ks - r.ks == 0.0f && r.vs - r.vs == 0.0f);
             r.ks = r.ks - r.ks == 0.0f ? r.ks : 1.0f;
-            r.vs = r.vs - r.vs == 0.0f ? __builtin_fmaxf(r.vs, 1.0e-37f) : 1.0e-37f;
-            r.e = eref = max(eref, __builtin_amdgcn_frexp_expf(r.vs));
+            r.vs = r.vs - r.vs == 0.0f ? __builtin_fmaxf(r.vs, kNoScale) : kNoScale;
+            const int own = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(r.vs));
+            eref = max(eref, own);
+            r.e = own >= eref - kExact || r.vs == kNoScale ? eref : max(own + kExact, eref - kDrop);
             return r;
         };
         struct Step {
@@ -272,8 +280,8 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
                 } else {
                     if (!values) continue;
                     const int d = (c - CH) >> 2, kch = (c - CH) & 3;
-                    const float ff = __builtin_amdgcn_ldexpf(1.0f, NH == 2 && (kch >> 1) ? f1 : f0);
-                    const f16 fh = (f16)ff, oh = (f16)(-1152.0f * ff);
+                    // rounded first: below 2^-24 the factor and the offset are zeros together
+                    const f16 fh = (f16)__builtin_amdgcn_ldexpf(1.0f, NH == 2 && (kch >> 1) ? f1 : f0), oh = (f16)-1152.0f * fh;
                     const f16x2 f2 = {fh, fh}, off = {oh, oh};
                     uint16_t* const row = vt[vslot] + d * kKB;
                     *reinterpret_cast<u32x4*>(row + 8 * swz<8>(d, 2 * kch)) = scaled_codes(reg.w[i][0], reg.w[i][2], f2, off);

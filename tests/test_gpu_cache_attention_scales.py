@@ -1,0 +1,99 @@
+"""GPU: attention over pages of the INT8 cache whose value scales are apart by far, or as large as the type holds.
+
+The bound of an output counts each key's own error alone: half an fp16 step of its softmax weight, or half the smallest step
+of fp16 where the weight is small, times that key's value; a weight that is below every step of fp16 is zero.  So a large
+value that a row hardly weighs buys no slack for the others.
+"""
+from __future__ import annotations
+
+import importlib
+
+import numpy as np
+import pytest
+import torch
+
+from _serving import LEAST, UNIT, Cache, f32, starts_of, tables
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+FP16, BF16 = torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def mod(pkg):
+    return importlib.import_module(f"{pkg.__name__}.opt.int8_kv_cache")
+
+
+def _int32(*arrays):
+    return [torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(DEV) for a in arrays]
+
+
+def _attend(ref, h, q, starts, lens, table, scale, causal, dtype):
+    """Head h of the cache for queries [tokens, dim], 64 bits -> (out, bound)."""
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    for b in range(len(lens)):
+        n, length = starts[b + 1] - starts[b], int(lens[b])
+        every = ref.keys_of(table, b, h, range(-(-length // ref.page)))
+        for i in range(n):
+            t = starts[b] + i
+            seen = length - n + i + 1 if causal else length
+            k, v = every[0][every[2] < seen], every[1][every[2] < seen]
+            x = q[t].astype(np.float64)
+            s = (k @ x) * scale
+            w = np.exp(s - s.max())
+            top = 1 / w.sum()                             # the largest weight
+            w *= top
+            out[t] = w @ v
+            # Weights are fp16 numbers of at least 2^6 (2^7 times the fraction of the value scale) and less than 2^15 for the
+            # largest weight: half a step is 2^-11 of a weight or 2^-25, and 2^-25 / 2^6 = 2^-31 of the largest; what is below
+            # 2^-25 / 2^15 = 2^-40 of it is less than half the smallest step and becomes zero (2^-42 here, for scores that are a little off).
+            # In the sum and in the product; scores and exp2 as in Cache.attend.
+            step = np.where(w < 2.0 ** -42 * top, w, np.maximum(2.0 ** -11 * w, 2.0 ** -31 * top))
+            slip = 2 * (ref.dim + 8) * 2.0 ** -24 * scale * float((np.abs(k) @ np.abs(x)).max()) + 2.0 ** -20
+            bound[t] = step @ np.abs(v) + step.sum() * np.abs(out[t]) + slip * (w @ np.abs(v))
+    return out, bound + UNIT[dtype] * np.abs(out) + LEAST[dtype]
+
+
+def _within(got, want, bound, what):
+    err = np.abs(got.double().cpu().numpy() - want)
+    bad = ~(err <= bound)
+    assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} past the bound, first at {np.argwhere(bad)[0].tolist()}, " \
+                          f"largest {np.nanmax(err / bound):.3g} of it"
+
+
+# exponents of the pages' value scales, the largest 0: codes that are exact next to those of the largest end at -24
+STEPS = (0, -24, -25, -26, -30, -35, -36, -2)
+FAR = (-60, 0, -31, -90, -47, -20, -70, -88)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,exponents,largest", [(FP16, STEPS, 8), (BF16, STEPS, 0), (BF16, FAR, 30)])
+@pytest.mark.parametrize("dim,page,kv", [(64, 32, 2), (64, 64, 2), (64, 128, 2), (128, 32, 1), (128, 64, 1), (128, 128, 1),
+                                         (64, 32, 96), (64, 64, 96), (64, 128, 96)])
+def test_rows_keep_the_values_of_their_own_page(mod, dtype, exponents, largest, dim, page, kv, causal):
+    """Every row's weight sits on one page, the pages' value scales are apart by up to 2^-90: rows of the small pages hold
+    those pages' values, in the long tiles (256 rows, and 512 with 96 kv heads) and in the 16-row tiles."""
+    pages = len(exponents)
+    new, lens = [200, 170], [pages * page, pages * page - 5]
+    table, pool = tables(lens, page, pages, seed=page + dim)
+    ref = Cache(pool, kv, dim, page, seed=dim)
+    rng = np.random.default_rng(90)
+    ref.k[:] = rng.integers(-2, 3, ref.k.shape)
+    ref.ks[:] = 1.0
+    for b in range(2):
+        for j, e in enumerate(exponents):
+            ref.k[table[b, j], :, :, j] = 100
+            ref.vs[table[b, j]] = 1.7 * 2.0 ** (largest + e) * (1 + 0.1 * (b + j % 3))
+    q = 0.3 * rng.standard_normal((sum(new), kv, dim))
+    for t in range(sum(new)):
+        q[t, :, :pages] = 0
+        q[t, :, t % pages] = 16.0                         # 100 x 16 x 1/8: 200 above the other pages' scores
+    q = torch.from_numpy(q).to(dtype)
+    starts = starts_of(new)
+    cache = ref.handle(mod, DEV)
+    ints = _int32(starts, lens, table)
+    h = kv - 1
+    want, bound = _attend(ref, h, f32(q[:, h]), starts, lens, table, 0.125, causal, dtype)
+    for hint in (1, None, 170):                           # 16-row tiles; both kernels; the long tiles alone
+        out = cache.attend(q.to(DEV), *ints, 0.125, causal=causal, max_new=hint)
+        _within(out[:, h], want, bound, f"max_new {hint}")
