@@ -184,7 +184,7 @@ __global__ __launch_bounds__(write_threads(D, P)) void kv_write_kernel(WritePara
             for (int off = LD; off < 64; off <<= 1) sum[e] += __builtin_bit_cast(s16x2, __shfl_xor(__builtin_bit_cast(int, sum[e]), off, 64));
             if (lane < LD) part[wave * (D / 2) + 4 * lane + e] = __builtin_bit_cast(int, sum[e]);
         }
-        if constexpr (NWV > 1) __syncthreads();
+        __syncthreads();   // also where one wave is the workgroup: its lanes read what other lanes wrote
         if (tid < D / 4) {
             s16x2 a = {0, 0}, c = {0, 0};      // dims 4 tid and + 2, + 1 and + 3
 #pragma unroll
