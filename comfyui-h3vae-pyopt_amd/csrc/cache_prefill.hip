@@ -49,6 +49,16 @@ __device__ __forceinline__ int swz(int row, int chunk) {
     else return chunk ^ (row & 15);
 }
 
+// Barrier of the workgroup's waves where the two halves of them run code of their own.  __syncthreads() may not stand there: it is
+// one place that all threads of a workgroup reach together.  s_barrier is an instruction of a wave: it waits until every wave of the workgroup
+// has come to one, wherever in the code that is.  Both halves come to 1 + steps of them per tile, and no branch of a wave's
+// lanes is around any; the fences are those of __syncthreads().
+__device__ __forceinline__ void halves_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+}
+
 // fp16 values of 8 codes times `f` (a power of two from 2^-24 on, or 0), exactly: (1024 + byte) f - 1152 f, with off = -1152 f
 __device__ __forceinline__ u32x4 scaled_codes(uint32_t w0, uint32_t w1, f16x2 f, f16x2 off) {
     const uint32_t u0 = w0 ^ 0x80808080u, u1 = w1 ^ 0x80808080u;
@@ -454,7 +464,7 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
             int slot = 0, up1 = 1, up2 = 2;                   // slots of j, j + 1, j + 2
             int pe0 = -126, pe1 = -126;
             auto sees = [&](int u) { return j0 * P + u * kKB < wave_last; };
-            __syncthreads();
+            halves_barrier();
             if (FIRST && AHEAD && sees(0)) scores(0);
             for (int j = 0; j < steps; ++j) {
                 store(next, j + 1 + AHEAD < steps, AHEAD ? up2 : up1, j + 1 < steps, s1, up1);
@@ -484,7 +494,7 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
                 slot = up1;
                 up1 = up2;
                 up2 = t;
-                __syncthreads();
+                halves_barrier();
             }
             if (!FIRST && sees(steps - 1)) product(pe0, pe1, up2);
         }
@@ -528,7 +538,8 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
                 }
         }
         };
-        // each half of the waves to the tile's end by itself: registers of the two need not agree anywhere
+        // each half of the waves to the tile's end by itself: registers of the two need not agree anywhere.  `wave` and `steps` are
+        // the same for all lanes of a wave, `steps` for all waves (halves_barrier)
         if (wave < NW / 2) work(std::true_type{});
         else work(std::false_type{});
         __syncthreads();   // the next tile's first store waits for this tile's last reads
