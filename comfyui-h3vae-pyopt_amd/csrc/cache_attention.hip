@@ -130,7 +130,7 @@ __global__ __launch_bounds__(kNT, 2) void cache_attention_kernel(AttnParams p) {
             }
             if (my_id >= 0) {
                 my_ks = p.ks[(int64_t)my_id * p.kv_heads + kvh];
-                my_vs = p.vs[(int64_t)my_id * p.kv_heads + kvh];
+                my_vs = p.vs[(int64_t)my_id * p.kv_heads + kvh] * (1.0f / (1 << kOutDrop));
             }
         };
         fetch(j0 + wave);

@@ -515,7 +515,7 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
                     for (int g = 0; g < 4; ++g) {
                         f32x4 v;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(o[qs][d][4 * g + e], oe);
+                        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(o[qs][d][4 * g + e], oe - kOutDrop);
                         *reinterpret_cast<f32x4*>(dst + 32 * d + 8 * g) = v;
                     }
                 if (hi == 0) {

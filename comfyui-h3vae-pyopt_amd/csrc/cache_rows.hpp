@@ -97,7 +97,7 @@ struct RowTile {
         }
     }
 
-    // the step of the keys key0 .., of which this lane's row sees those below `seen`
+    // the step of the keys key0 .., of which this lane's row sees those below `seen`; vs: the page's value scale times 2^-kOutDrop
     __device__ __forceinline__ void attend(const Codes& w, int key0, float ks, float vs, int seen) {
         // a factor that is too small for fp32 keeps a masked score at minus infinity
         const float kc = ks * c < 1.0e-37f ? 1.0e-37f : ks * c;
@@ -233,8 +233,10 @@ struct Joined {
     }
 };
 
-// Reciprocal of a row's sum; a row that saw no key gets 0.
-__device__ __forceinline__ float row_inverse(float top, float sum) { return top == -kInf && sum == 0.0f ? 0.0f : 1.0f / sum; }
+// What brings a row's unnormalised output to its value: 2^kOutDrop over the row's sum; a row that saw no key gets 0.
+__device__ __forceinline__ float row_inverse(float top, float sum) {
+    return top == -kInf && sum == 0.0f ? 0.0f : (float)(1 << kOutDrop) / sum;
+}
 
 template <int DT>
 __device__ __forceinline__ void put_row(uint16_t* at, const f32x4& v, float inv) {

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(kNT, D == 64 ? 3 : 2) void cache_selected_kernel(Se
                 }
                 if (my_id >= 0) {
                     my_ks = p.ks[(int64_t)my_id * p.kv_heads + kvh];
-                    my_vs = p.vs[(int64_t)my_id * p.kv_heads + kvh];
+                    my_vs = p.vs[(int64_t)my_id * p.kv_heads + kvh] * (1.0f / (1 << kOutDrop));
                 }
                 struct Step {
                     typename Tile::Codes codes;

@@ -25,7 +25,7 @@ def mod(pkg):
 
 
 def _int32(*arrays):
-    return [torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(DEV) for a in arrays]
+    return [torch.from_numpy(np.array(a, dtype=np.int32)).to(DEV) for a in arrays]
 
 
 def _attend(ref, h, q, starts, lens, table, scale, causal, dtype):
@@ -97,3 +97,31 @@ def test_rows_keep_the_values_of_their_own_page(mod, dtype, exponents, largest, 
     for hint in (1, None, 170):                           # 16-row tiles; both kernels; the long tiles alone
         out = cache.attend(q.to(DEV), *ints, 0.125, causal=causal, max_new=hint)
         _within(out[:, h], want, bound, f"max_new {hint}")
+
+
+@pytest.mark.parametrize("codes", ["largest", "random"])
+@pytest.mark.parametrize("dim,page,kv,group,new,held,width", [
+    (64, 64, 2, 2, 1, 500, 8), (128, 32, 1, 4, 1, 5000, 157), (128, 128, 2, 1, 3, 300, 4),     # 16-row tiles, one split and several
+    (64, 64, 1, 4, 100, 300, 8), (128, 32, 1, 2, 120, 2000, 70), (64, 64, 64, 1, 300, 3, 6)])  # long tiles likewise
+def test_values_near_the_largest_of_bf16(mod, codes, dim, page, kv, group, new, held, width):
+    """Outputs are averages of values, finite where the values are: sums of up to thousands of the largest that bf16 holds, over
+    all keys and over selected pages (a token to a workgroup, and several)."""
+    lens = [new + held]
+    pages = -(-lens[0] // page)
+    table, pool = tables(lens, page, width, seed=page + dim)
+    ref = Cache(pool, kv, dim, page, seed=dim)
+    if codes == "largest":
+        ref.v[:] = 127
+    ref.vs[:] = 3.38e38 / 127
+    rng = np.random.default_rng(92)
+    q = torch.from_numpy(rng.standard_normal((new, kv * group, dim))).to(BF16)
+    cache = ref.handle(mod, DEV)
+    starts = starts_of([new])
+    ints = _int32(starts, lens, table)
+    lists = np.broadcast_to(np.arange(pages, dtype=np.int32), (new, kv, pages))
+    outs = {"all": cache.attend(q.to(DEV), *ints, dim ** -0.5),
+            "selected": cache.attend_selected(q.to(DEV), *_int32(lists), *ints, dim ** -0.5)}
+    for what, out in outs.items():
+        for h in {0, kv * group - 1}:
+            want, bound = _attend(ref, h // group, f32(q[:, h]), starts, lens, table, dim ** -0.5, True, BF16)
+            _within(out[:, h], want, bound, what)
