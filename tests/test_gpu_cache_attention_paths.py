@@ -20,7 +20,7 @@ def mod(pkg):
 
 
 def _int32(*arrays):
-    return [torch.from_numpy(np.array(a, dtype=np.int32)).to(DEV) for a in arrays]
+    return [torch.from_numpy(np.array(a, dtype=np.int32, order="C")).to(DEV) for a in arrays]
 
 
 def _queries(tokens, heads, dim, dtype, seed):
