@@ -11,6 +11,10 @@ constexpr float kLazy = 8.0f;         // log2 margin of the lazy softmax maximum
 // the reference keep all their bits: many keys far below one that stands out lose nothing of their sum.  The sums carry the
 // same factor, which the division takes out.
 constexpr float kLift = 7.0f;
+// References up to here: the exponent of a weight is one fma of score, factor and reference, which carries the product's bits that
+// the reference, a rounded maximum, has lost, half a unit at most: weights stay within 2^15.5.  Beyond, where such
+// bits would be whole powers of two, the product is rounded as the maximum was.
+constexpr float kFar = 4194304.0f;
 // Unnormalised outputs, in registers and in the workspace, are 2^-kOutDrop of what they stand for, which the last division takes
 // back.  A bf16 value goes up to 2^128, and the sum of its weights (at most 2^15 each, 2^7 at the maximum) would pass fp32's
 // range; with 2^-26 it may be 2^26, 2^19 keys at the maximum.  The least scale, 1e-30, stays a normal number.

@@ -311,6 +311,7 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
             m[qs] = -kInf;
             l[qs] = 0.0f;
         }
+        bool far = false;                                    // some row's reference is past kFar (the same for all lanes)
         uint32_t pk[QS][2][8];
 
         f32x16 x[QS][2];
@@ -376,6 +377,7 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
                 up |= top[qs] > m[qs] + kLazy;
             }
             if (__ballot(up)) {
+                bool past = false;
 #pragma unroll
                 for (int qs = 0; qs < QS; ++qs) {
                     const float m_new = __builtin_fmaxf(m[qs], __builtin_fmaxf(top[qs], __shfl_xor(top[qs], 32, 64)));
@@ -384,11 +386,26 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
                     l[qs] *= alpha;
 #pragma unroll
                     for (int d = 0; d < DB; ++d) o[qs][d] *= alpha;
+                    past |= __builtin_fabsf(m[qs]) > kFar && m[qs] > -kInf;
                 }
+                far = __ballot(past) != 0;
+            }
+            if (far) {                                       // weights from rounded scores less the reference
+#pragma unroll
+                for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+                    for (int kh = 0; kh < 2; ++kh) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[qs][kh][r] = x[qs][kh][r] * kf[qs][NH == 2 ? kh : 0] - (m[qs] == -kInf ? 0.0f : m[qs]);
+                    }
+#pragma unroll
+                for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) kf[qs][h] = 1.0f;
             }
 #pragma unroll
             for (int qs = 0; qs < QS; ++qs) {
-                const float base = (m[qs] == -kInf ? 0.0f : m[qs]) - kLift;
+                const float base = (far || m[qs] == -kInf ? 0.0f : m[qs]) - kLift;
                 float sum = 0.0f;
 #pragma unroll
                 for (int kh = 0; kh < 2; ++kh) {

@@ -33,6 +33,7 @@ struct RowTile {
     f32x4 o[ND];
     float add, l;          // the exponents' addend: kLift minus the reference maximum (infinite without one); the row's sum
     bool any;              // this lane's row saw a key
+    bool far;              // some row's reference is past kFar (the same for all lanes)
 
     // row: the query row of this lane's column.  Only loads; set_rows() makes fragments of them.
     __device__ __forceinline__ void load_rows(const uint16_t* row) {
@@ -49,6 +50,7 @@ struct RowTile {
         add = kInf;
         l = 0.0f;
         any = false;
+        far = false;
     }
 
     __device__ __forceinline__ void set_rows(float scale) {
@@ -134,12 +136,19 @@ struct RowTile {
             const float lower = __builtin_fminf(add, kLift - top);
             const float alpha = add == lower ? 1.0f : __builtin_amdgcn_exp2f(lower - add);
             add = lower;
+            far = __ballot(__builtin_fabsf(add) > kFar && add < kInf) != 0;
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] *= alpha;
         }
         // a row that sees no key of the step takes nothing from it, not even from a scale that is NaN
-        const float factor = sees ? kc : 1.0f, from = sees ? add : -kInf, vrow = sees ? vs : 0.0f;
+        float factor = sees ? kc : 1.0f;
+        const float from = sees ? add : -kInf, vrow = sees ? vs : 0.0f;
+        if (far) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) x[t] *= factor;
+            factor = 1.0f;
+        }
         uint32_t pk[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {

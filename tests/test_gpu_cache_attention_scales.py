@@ -125,3 +125,45 @@ def test_values_near_the_largest_of_bf16(mod, codes, dim, page, kv, group, new, 
         for h in {0, kv * group - 1}:
             want, bound = _attend(ref, h // group, f32(q[:, h]), starts, lens, table, dim ** -0.5, True, BF16)
             _within(out[:, h], want, bound, what)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype,dim,page,kv,group,new,held,width", [
+    (FP16, 64, 64, 2, 2, 1, 500, 8), (BF16, 128, 32, 1, 4, 1, 5000, 157), (FP16, 128, 128, 2, 1, 3, 300, 4),   # 16-row tiles
+    (FP16, 64, 64, 1, 4, 100, 300, 8), (BF16, 128, 32, 1, 2, 120, 2000, 70), (FP16, 64, 32, 64, 1, 300, 3, 10)])  # long tiles
+def test_scores_of_many_millions(mod, sign, dtype, dim, page, kv, group, new, held, width):
+    """Scores of 1e7 to 1e11, where a step of fp32 is many times the softmax's unit, all positive or all negative: the key that
+    stands out has the whole weight; rows of common size beside them keep their accuracy."""
+    lens = [new + held]
+    pages = -(-lens[0] // page)
+    table, pool = tables(lens, page, width, seed=page + dim)
+    ref = Cache(pool, kv, dim, page, seed=dim)
+    rng = np.random.default_rng(93)
+    ref.k[:] = rng.integers(30, 128, ref.k.shape)
+    ref.ks[:] = (400 + 100 * rng.random(ref.ks.shape)).astype(np.float32)
+    sizes = np.exp(rng.uniform(np.log(30), np.log(6e4), (new, kv * group, 1)))
+    small = rng.random((new, kv * group, 1)) < 0.3
+    sizes[small] = 1e-6 / dim
+    q = torch.from_numpy(sign * sizes * (0.5 + 0.5 * rng.random((new, kv * group, dim)))).to(dtype)
+    cache = ref.handle(mod, DEV)
+    starts = starts_of([new])
+    ints = _int32(starts, lens, table)
+    lists = np.broadcast_to(np.arange(pages, dtype=np.int32), (new, kv, pages))
+    outs = {"all": cache.attend(q.to(DEV), *ints, 0.125),
+            "selected": cache.attend_selected(q.to(DEV), *_int32(lists), *ints, 0.125)}
+    for h in {0, kv * group - 1}:
+        want, bound = _attend(ref, h // group, f32(q[:, h]), starts, lens, table, 0.125, True, dtype)
+        clear = np.ones(new, bool)
+        k, v, pos = ref.keys_of(table, 0, h // group, range(pages))
+        for t in range(new):
+            if small[t, h, 0]:
+                continue
+            s = np.sort((k[pos <= held + t] @ f32(q[t, h]).astype(np.float64)) * 0.125)
+            # fp32 sums of dim exact products are within (dim + 8) 2^-24 of the largest: a key further ahead than
+            # twice that and 200 has every other's weight at zero
+            clear[t] = len(s) < 2 or s[-1] - s[-2] > 2 * (dim + 8) * 2.0 ** -24 * np.abs(s).max() + 200
+            bound[t] = (2.0 ** -10 + UNIT[dtype]) * np.abs(want[t]) + LEAST[dtype]
+        assert new == 1 or clear.sum() > new / 2
+        for what, out in outs.items():
+            _within(out[:, h][torch.from_numpy(clear).to(DEV)], want[clear], bound[clear], what)
+            assert torch.isfinite(out[:, h]).all(), what
