@@ -74,11 +74,12 @@ __device__ __forceinline__ u32x4 scaled_codes(uint32_t w0, uint32_t w1, f16x2 f,
 // One page's part of a step: its id (-1: not there) and scales.  A value scale of zero (its codes are) or a bad scale (infinite
 // or NaN: the scores of the rows that see the page become NaN) stands as a harmless number.
 constexpr float kNoScale = 1.0e-37f;
+constexpr int kNoExponent = -122;
 struct Part {
     int id;
     float ks, vs;
     bool bad;
-    int e;        // the reference exponent of its codes and of the accumulators
+    int e, f;     // the reference exponent of the codes and of the accumulators, and what the codes have on top of it
 };
 
 // Codes are exact down to 2^-24 of the reference.  It drops by at most 75: accumulators stay below 2^(kLazy + kLift) * 127 * 2^30 keys
@@ -209,8 +210,9 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
         }
 
         // pages of the split, 64 at a time: ids and scales one page per lane
-        int pg_base = -64, pg_id = -1;
+        int pg_base = -64, pg_id = -1, pg_e = 0;              // pg_e: exponent of the value scale, kBadPage more where a scale is bad
         float pg_ks = 0.0f, pg_vs = 0.0f;
+        constexpr int kBadPage = 4096;
         int eref = -126;                                      // largest value exponent of the steps so far
         auto part_of = [&](int j) {                           // page j0 + j
             if (j - pg_base >= 64) {
@@ -222,18 +224,22 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
                     pg_ks = p.ks[(int64_t)pg_id * p.kv_heads + kvh];
                     pg_vs = p.vs[(int64_t)pg_id * p.kv_heads + kvh];
                 }
+                const bool bad = !(pg_ks - pg_ks == 0.0f && pg_vs - pg_vs == 0.0f);
+                pg_ks = pg_ks - pg_ks == 0.0f ? pg_ks : 1.0f;
+                pg_vs = pg_vs - pg_vs == 0.0f ? __builtin_fmaxf(pg_vs, kNoScale) : kNoScale;
+                pg_e = __builtin_amdgcn_frexp_expf(pg_vs) + (bad ? kBadPage : 0);
             }
             const int n = j - pg_base;
             Part r;
             r.id = __builtin_amdgcn_readlane(pg_id, n);
             r.ks = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, pg_ks), n));
             r.vs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, pg_vs), n));
-            r.bad = !(r.ks - r.ks == 0.0f && r.vs - r.vs == 0.0f);
-            r.ks = r.ks - r.ks == 0.0f ? r.ks : 1.0f;
-            r.vs = r.vs - r.vs == 0.0f ? __builtin_fmaxf(r.vs, kNoScale) : kNoScale;
-            const int own = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(r.vs));
+            const int e = __builtin_amdgcn_readlane(pg_e, n);
+            r.bad = e > kBadPage / 2;
+            const int own = r.bad ? e - kBadPage : e;
             eref = max(eref, own);
-            r.e = own >= eref - kExact || r.vs == kNoScale ? eref : max(own + kExact, eref - kDrop);
+            r.e = own >= eref - kExact || own == kNoExponent ? eref : max(own + kExact, eref - kDrop);
+            r.f = own - r.e;
             return r;
         };
         struct Step {
@@ -275,8 +281,7 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
             }
         };
         auto store = [&](const Chunks& reg, bool keys, int kslot, bool values, const Step& sv, int vslot) {
-            const int f0 = __builtin_amdgcn_frexp_expf(sv.h[0].vs) - sv.h[0].e;
-            const int f1 = NH == 2 ? __builtin_amdgcn_frexp_expf(sv.h[NH - 1].vs) - sv.h[NH - 1].e : f0;
+            const int f0 = sv.h[0].f, f1 = sv.h[NH - 1].f;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const int c = tid + i * NT;
