@@ -31,16 +31,25 @@ struct NormParams {
     float* scale;
 };
 
-template <int W>
-__device__ __forceinline__ float row_sum(float v, float* red, int wave) {
+__device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-    if constexpr (W > 1) {
-        if ((threadIdx.x & 63) == 0) red[wave] = v;
-        __syncthreads();
-        v = (red[0] + red[1]) + (red[2] + red[3]);
-    }
     return v;
+}
+
+// Sum over a row of the lanes' sums.  One wave: a sum for each of up to two chunks, joined as two waves would join theirs, so that a
+// row's bits do not depend on how many waves it has.
+template <int W, int N>
+__device__ __forceinline__ float row_sum(const float (&v)[N], float* red, int wave) {
+    static_assert(W == 1 ? N <= 2 : N == 1);
+    const float s = wave_sum(v[0]);
+    if constexpr (W > 1) {
+        if ((threadIdx.x & 63) == 0) red[wave] = s;
+        __syncthreads();
+        return (red[0] + red[1]) + (red[2] + red[3]);
+    }
+    if constexpr (N > 1) return s + wave_sum(v[N - 1]);
+    return s;
 }
 
 // How a call uses the caches, by the bytes of its outputs (gated norms alone / with a sum and a matrix product that read h and n,
@@ -88,20 +97,21 @@ __global__ __launch_bounds__(kNT) void gated_norms_kernel(NormParams p) {
             xw[c] = yw[c] = gw[c] = u32x4{0, 0, 0, 0};
         }
     }
+    constexpr int NS = W == 1 ? NCH : 1;                 // sums of a lane
     float f = p.alpha;
     if constexpr (POST) {
-        float ss = 0.0f;
+        float ss[NS] = {};
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
             float v[8];
             unpack8<DT>(yw[c], v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(v[e], v[e], ss);
+            for (int e = 0; e < 8; ++e) ss[c % NS] = __builtin_fmaf(v[e], v[e], ss[c % NS]);
         }
         f *= rsqrt_rn(row_sum<W>(ss, red[0], wave) * inv_k + p.eps);
     }
     float h[NCH][8];
-    float ss = 0.0f;
+    float ss[NS] = {};
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
         float xv[8], yv[8], gv[8], wv[8];
@@ -114,7 +124,7 @@ __global__ __launch_bounds__(kNT) void gated_norms_kernel(NormParams p) {
             float z = yv[e] * f;
             if (POST) z *= col[c] < p.k ? wv[e] : 0.0f;
             h[c][e] = gate ? __builtin_fmaf(z, gv[e], xv[e]) : xv[e] + z;
-            ss = __builtin_fmaf(h[c][e], h[c][e], ss);
+            ss[c % NS] = __builtin_fmaf(h[c][e], h[c][e], ss[c % NS]);
         }
         if (col[c] < p.k) write_out<USE != Use::Plain>(p.h + base + col[c], pack8<DT>(h[c]));
     }
@@ -180,9 +190,17 @@ void launch(const NormParams& p, hipStream_t stream) {
 
 constexpr int64_t kMaxWidth = 16384;
 
+// Waves of a row.  One wave holds up to 512 values in a chunk and joins nothing in LDS; four share wider rows.  From 513 to
+// 1024 four waves leave up to half of themselves idle, which counts once the rows fill the chip (us, one wave / four, fp16
+// out): 7188 x 64 5.9 / 12.5, 7188 x 512 6.8 / 13.1; 8 x 1024 4.1 / 3.6, 700 x 1024 4.4 / 4.2, 1024 x 1024 4.8 / 4.8, 1400 x 1024
+// 5.0 / 5.5, 7188 x 1024 11.3 / 16.0, 7188 x 520 8.9 / 14.1; int8 rows 700 x 1024 4.7 / 4.6, 1024 x 1024 4.9 / 5.3, 7188 x 1024
+// 12.3 / 17.9; 512 x 2048 6.2 / 4.4, 7188 x 2048 23.8 / 23.0.
+constexpr int64_t kOneWaveRows = 1024;
+
 template <int DT>
 void dispatch(const NormParams& p, hipStream_t stream) {
     if (p.k <= 512) launch<DT, 1, 1>(p, stream);
+    else if (p.k <= 1024 && p.m >= kOneWaveRows) launch<DT, 1, 2>(p, stream);
     else if (p.k <= 2048) launch<DT, 4, 1>(p, stream);
     else if (p.k <= 4096) launch<DT, 4, 2>(p, stream);
     else if (p.k <= 8192) launch<DT, 4, 4>(p, stream);
