@@ -245,7 +245,12 @@ __global__ __launch_bounds__(write_threads(D, P)) void kv_write_kernel(WritePara
     }
 }
 
-constexpr int64_t kL2Bytes = 32 << 20;
+// A read's outputs are stored past the L2s where they fit there with room for a reader's own, so that none are left to write back at
+// the kernel's end, and where they are more than the Infinity Cache holds; between, they are left there for their reader. us, plain /
+// streamed, alone and with a sum that reads them: 12 MB 5.6 / 4.7, 12.9 / 12.2; 17 MB 7.1 / 5.7, 15.7 / 14.8; 20.5 MB 7.5 / 5.3, 17.2 /
+// 17.1; 24 MB 8.3 / 5.8, 18.2 / 18.8; 31 MB 9.3 / 8.4, 18.7 / 20.1; 59 MB 15.6 / 15.6, 29.3 / 30.7; 197 MB 48 / 45, 94 / 105; 328 MB
+// 97 / 91, 182 / 177; 655 MB 191 / 179, 358 / 350.
+constexpr int64_t kStreamBelow = 20 << 20, kStreamAbove = 256 << 20;
 
 struct ReadParams {
     Sequences s;
@@ -256,8 +261,7 @@ struct ReadParams {
     int heads, length;
 };
 
-// STREAM: outputs that the L2s hold together are stored past them, so that none are left to write back at the kernel's end;
-// larger ones are left to the Infinity Cache, where their reader finds them.
+// STREAM: outputs are stored past the L2s.
 template <int DT, int D, int P, bool STREAM>
 __global__ __launch_bounds__(read_threads(D, P)) void kv_read_kernel(ReadParams p) {
     constexpr int NT = read_threads(D, P), NU = units_of(D, P) / NT;
@@ -394,8 +398,10 @@ int h3v_kv_cache_read(int dtype, const int8_t* k_cache, const int8_t* v_cache, c
     const int64_t tiles = (length / page + 2) * heads;
     H3V_REQUIRE(tiles * 256 <= 0xffffffffll, "%s: too long", what);
     const dim3 grid((unsigned)tiles, 1, (unsigned)(2 * batch));
+    const int64_t bytes = 4 * batch * length * heads * dim;
+    const bool stream_out = bytes <= kStreamBelow || bytes > kStreamAbove;
     by_shape(dtype, dim, page, [&](auto dt, auto d, auto pg) {
-        if (4 * batch * length * heads * dim <= kL2Bytes) hipLaunchKernelGGL((kv_read_kernel<dt(), d(), pg(), true>), grid, dim3(read_threads(d(), pg())), 0, stream, p);
+        if (stream_out) hipLaunchKernelGGL((kv_read_kernel<dt(), d(), pg(), true>), grid, dim3(read_threads(d(), pg())), 0, stream, p);
         else hipLaunchKernelGGL((kv_read_kernel<dt(), d(), pg(), false>), grid, dim3(read_threads(d(), pg())), 0, stream, p);
     });
     return launch_status(what);

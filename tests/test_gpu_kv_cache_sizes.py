@@ -1,4 +1,4 @@
-"""GPU: the key means that a write leaves, of pages that one wave writes and of pages that several do, equal to the means of
+"""GPU: reads of every size; and the key means that a write leaves, of pages that one wave writes and that several do, against those of
 the codes that it left."""
 from __future__ import annotations
 
@@ -34,3 +34,22 @@ def test_key_means_are_those_of_the_codes(pkg, dtype, dim, page):
                 p = int(table[b, j])
                 total = codes[p, :, :held].sum(1, dtype=torch.int32)
                 assert torch.equal(means[p], (total.float() / held).round().to(torch.int8)), (b, j)
+
+
+@pytest.mark.parametrize("length", [3700, 5300, 70000])
+def test_reads_of_every_size_are_the_codes_times_the_scale(pkg, length):
+    """Outputs that are stored past the caches (15 and 287 MB) and that are left in them (22 MB): one batch of shared pages, bit for bit."""
+    kv = importlib.import_module(f"{pkg.__name__}.opt.int8_kv_cache")
+    heads, dim, page, pool = 8, 128, 64, 50
+    gen = torch.Generator().manual_seed(length)
+    k = torch.randint(-127, 128, (pool, heads, page, dim), generator=gen, dtype=torch.int8).to(DEV)
+    v = torch.randint(-127, 128, (pool, heads, dim, page), generator=gen, dtype=torch.int8).to(DEV)
+    ks, vs = (torch.rand(pool, heads, generator=gen).to(DEV) for _ in range(2))
+    cache = kv.Int8KVCache(k, v, ks, vs, torch.zeros((pool, heads, dim), dtype=torch.int8, device=DEV))
+    table = torch.randint(0, pool, (1, -(-length // page)), generator=gen).int().to(DEV)
+    ints = [torch.tensor([n], dtype=torch.int32, device=DEV) for n in (0, length)]
+    got = cache.read(*ints, table, length)
+    ids = table[0].long()
+    for out, codes, scale in ((got[0], k, ks), (got[1], v.transpose(2, 3), vs)):
+        want = (codes[ids].float() * scale[ids][..., None, None]).half().transpose(1, 2).reshape(-1, heads, dim)[:length]
+        assert torch.equal(out[0], want)
