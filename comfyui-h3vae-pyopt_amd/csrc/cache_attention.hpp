@@ -66,6 +66,9 @@ __device__ __forceinline__ int keys_seen(const AttnParams& p, const Span& sp, in
     return n > 0 ? (int)n : 0;
 }
 
+// a reference past kFar; a row without one, or with an infinite score, whose result is NaN, has none
+__device__ __forceinline__ bool is_far(float reference) { return __builtin_fabsf(reference) > kFar && __builtin_fabsf(reference) < kInf; }
+
 // merge weight of a part with reference maximum m under the common maximum top
 __device__ __forceinline__ float part_weight(float m, float top) {
     return m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);

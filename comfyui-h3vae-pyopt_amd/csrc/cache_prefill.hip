@@ -391,7 +391,7 @@ __global__ __launch_bounds__(64 * kNW) void cache_prefill_kernel(AttnParams p) {
                     l[qs] *= alpha;
 #pragma unroll
                     for (int d = 0; d < DB; ++d) o[qs][d] *= alpha;
-                    past |= __builtin_fabsf(m[qs]) > kFar && m[qs] > -kInf;
+                    past |= is_far(m[qs]);
                 }
                 far = __ballot(past) != 0;
             }

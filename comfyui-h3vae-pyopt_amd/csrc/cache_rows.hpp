@@ -136,7 +136,7 @@ struct RowTile {
             const float lower = __builtin_fminf(add, kLift - top);
             const float alpha = add == lower ? 1.0f : __builtin_amdgcn_exp2f(lower - add);
             add = lower;
-            far = __ballot(__builtin_fabsf(add) > kFar && add < kInf) != 0;
+            far = __ballot(is_far(add)) != 0;
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] *= alpha;

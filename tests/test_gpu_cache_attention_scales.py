@@ -167,3 +167,26 @@ def test_scores_of_many_millions(mod, sign, dtype, dim, page, kv, group, new, he
         for what, out in outs.items():
             _within(out[:, h][torch.from_numpy(clear).to(DEV)], want[clear], bound[clear], what)
             assert torch.isfinite(out[:, h]).all(), what
+
+
+@pytest.mark.parametrize("hint", [None, 1])
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_an_infinite_query_changes_no_bit_of_the_rows_beside_it(mod, dtype, hint):
+    """Its row is NaN; the others' weights are made as without it, in the long tiles and in tiles of 16 rows."""
+    heads, dim, page, new, held = 2, 64, 64, 192, 900
+    table, pool = tables([held + new], page, 18, seed=4)
+    ref = Cache(pool, heads, dim, page, seed=5)
+    ref.k[..., 0], ref.ks[:] = 127, 0.5
+    cache = ref.handle(mod, DEV)
+    # scores of 5e5, all nearly alike: a step of fp32 there is a sixteenth, which other roundings would show
+    q = torch.randn(new, heads, dim, generator=torch.Generator().manual_seed(6)).to(dtype)
+    q[..., 0] = 6e4
+    q[::16] = 0
+    ints = _int32([0, new], [held + new], table)
+    want = cache.attend(q.to(DEV), *ints, 0.125, max_new=hint)
+    bad = q.clone()
+    bad[::16, :, 0] = float("inf")                        # an infinite score of every key
+    out = cache.attend(bad.to(DEV), *ints, 0.125, max_new=hint)
+    rows = [t for t in range(new) if t % 16]
+    assert torch.isnan(out[::16]).all()
+    assert torch.equal(out[rows], want[rows])
