@@ -25,9 +25,9 @@
 // order costs 2 to 10%.)  Between barriers j and j + 1 every wave stores its part of the values of step j + 1 and of the keys of step
 // j + 1 or, where scores are ahead, j + 2, and loads those after them; the slots they go into were last read before barrier j.
 //
-// 4 x 1797 over 7188, 32 heads of 64: 417 us, 800 TFLOP/s, of the 252 us that a library matrix product of as many operations
-// takes.  The vector units are busy for 61% of the time and the matrix units for 35%; without the staging of codes into
-// fp16 it would be 352, without the exponentials 388.  1 x 4096 over 8192, 32 heads of 128: 568 us, 970 TFLOP/s.
+// 4 x 1797 over 7188, 32 heads of 64: 404 to 420 us, 800 TFLOP/s, where a library matrix product of as many operations
+// takes 252.  The vector units are busy for 58% of the time and the matrix units for 35%; without the staging of codes into
+// fp16 it would be 352, without the exponentials 388.  1 x 4096 over 8192, 32 heads of 128: 560 us, 980 TFLOP/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -580,9 +580,9 @@ void launch_shape(const AttnParams& p, dim3 grid, hipStream_t stream) {
 
 }  // namespace
 
-// At dim 64 two sets of 32 rows per wave read each key and value fragment once for both, but a CU holds one such workgroup:
-// they pay where they make two rounds on the 256 CUs, or fill one without causal rows, whose longest tile would be the
-// round (us, 512 / 256 rows; batch x new over length, 32 heads):
+// At dim 64 two sets of 32 rows per wave read each key and value fragment once for both.  A CU holds one workgroup of either
+// form (by the registers of its 8 waves), so there have to be twice the rows: the larger one pays where it makes two rounds on the
+// 256 CUs, or fills one without causal rows, whose longest tile would be the round (us, 512 / 256 rows; batch x new over length, 32 heads):
 //   4 x 1797 over 7188: 413 / 513, causal 373 / 445;  1 x 4096: 160 / 194, causal 148 / 110;  3 x 1100: 85 / 64, causal 57 / 53
 //
 // The keys are split where that shortens the rounds by more than the splits' outputs cost, written and joined (4 TB/s and a

@@ -497,7 +497,8 @@ int h3v_cache_select(int dtype, const uint16_t* q, int64_t q_token_stride, int64
                      int64_t blocks, int64_t sink, int64_t local, int* selected, hipStream_t stream);
 
 /* Attention over those pages alone, keys up to the token's own position.  selected: any logical pages in any order; an
- * entry outside the sequence is skipped, one named twice counts twice.  At most 16 heads per kv head. */
+ * entry outside the sequence is skipped, one named twice counts twice.  At most 16 heads per kv head.  The workspace is that of single
+ * tokens, at most 4.3 MB; where a sequence has several tokens the call may leave it unused. */
 int64_t h3v_cache_attention_selected_workspace_floats(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t blocks);
 int h3v_cache_attention_selected(int dtype, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
                                  const int* selected, int64_t blocks, const int* starts, const int* lens, const int* table,
